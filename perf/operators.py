@@ -9,7 +9,6 @@ A case is a dict of plain values; `kind` names the operator:
 
 With `own` false a pass computes the operators' definitions with elementary torch operations in 32 bits.
 """
-import functools
 import math
 import os
 import sys
@@ -24,9 +23,8 @@ DTYPES = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
 DENSE = ((5120, 8192), (4608, 5120), (32768, 1280), (1280, 5120), (5120, 2304), (3328, 7168), (7168, 1664), (8192, 8192))
 
 
-@functools.lru_cache(maxsize=None)
 def _ops():
-    """The framework's modules (where `own` is true), looked up once, as a program's imports are."""
+    """The framework's modules (where `own` is true)."""
     pkg = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "deepseekv4.1-a100-custom_amd")
     if pkg not in sys.path:
         sys.path.insert(0, pkg)
