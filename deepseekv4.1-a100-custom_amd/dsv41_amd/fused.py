@@ -61,13 +61,14 @@ NORM_MAX = 32768   # longest row of add_rmsnorm_quant (csrc/mx.h)
 _BITS = {"fp8": 8, "fp4": 4}
 
 
-def _apart(out: torch.Tensor, t: torch.Tensor) -> bool:
-    """Whether the rows of out share no byte with those of t, or are the same rows exactly (matrices of one type, as the kernel walks them)."""
+def _apart(out: torch.Tensor, t: torch.Tensor, same: bool = True) -> bool:
+    """Whether the rows of out share no byte with those of t, or are the same rows exactly where `same` allows it (matrices of one type, as
+    the kernel walks them)."""
     es, n = out.element_size(), out.shape[1] * out.element_size()
     so, st = _lib.row_stride(out) * es, _lib.row_stride(t) * es
     a, b = out.data_ptr(), t.data_ptr()
     if a == b and so == st and out.shape == t.shape:
-        return True
+        return same
     if a + (out.shape[0] - 1) * so + n <= b or b + (t.shape[0] - 1) * st + n <= a:
         return True
     return so == st and n <= (a - b) % so <= so - n   # other columns of the same wider rows
@@ -141,6 +142,7 @@ def _norm_rows(x, residual, w, out, K: int):
             o2 = None
         if o2 is None or (o2.shape[0] and _rows16(o2, es) is not o2):
             raise ValueError("out needs rows of 16-byte pieces in one regular layout (unit stride within a row, aligned rows)")
-        if not all(_apart(o2, t) for t in (x2, r2, w.view(1, K))):
+        # each value of x and the residual is read by the thread that writes r there; w is read by every row, after r is written
+        if not (_apart(o2, x2) and _apart(o2, r2) and _apart(o2, w.view(1, K), same=False)):
             raise ValueError("out overlaps an input without being it")
     return ((x2, r2, w), x2.data_ptr(), w.data_ptr(), r2.data_ptr(), o2.data_ptr(), _lib.row_stride(x2), _lib.row_stride(r2), _lib.row_stride(o2), out)

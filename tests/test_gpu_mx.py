@@ -672,3 +672,15 @@ def test_streams_and_graph():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(want, out))
+
+
+def test_add_rmsnorm_quant_refuses_the_weight_as_output():
+    """One row: `out` of the weight's shape may be x or the residual, not the weight, which is left as it was."""
+    from dsv41_amd import fused
+    g = gen(41)
+    x, res, w = (randn(g, *s, dtype=torch.bfloat16).cuda() for s in ((1, 5120), (1, 5120), (5120,)))
+    keep, want = w.clone(), fused.add_rmsnorm_quant(x, res, w, 1e-6)
+    with pytest.raises(ValueError, match="overlaps"):
+        fused.add_rmsnorm_quant(x, res, w, 1e-6, out=w.view(1, 5120))
+    assert torch.equal(w, keep)
+    assert all(torch.equal(a, b) for a, b in zip(want, fused.add_rmsnorm_quant(x, res, w, 1e-6, out=x)))

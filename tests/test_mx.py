@@ -184,3 +184,16 @@ def test_c_entries_refuse_without_launch():
                 dict(K=80), dict(M=-1), dict(fmt=0), dict(dtype=3), dict(out_type=3), dict(ldx=64), dict(ldx=100), dict(ldy=63), dict(x=q), dict(plan=4),
                 dict(plan=3, M=17), dict(plan=3, M=16, K=16384, ldx=16384)):
         assert linear(**bad) == -1, bad
+
+
+@pytest.mark.parametrize("rows", [1, 2])
+def test_norm_output_is_never_the_weight(rows):
+    """`out` may be x or the residual, not the weight: the kernel reads it after r is written. One row has the weight's own shape."""
+    from dsv41_amd import fused
+    x, res, w = torch.zeros(rows, 64), torch.zeros(rows, 64), torch.ones(64)
+    for out in (x, res):
+        assert fused._norm_rows(x, res, w, out, 64)[-1] is out
+    buf = torch.ones(4 * 64)
+    for w, out in ((w, w.view(1, 64).expand(rows, 64)), (buf[:64], buf[:rows * 64].view(rows, 64)), (buf[32:96], buf[:rows * 64].view(rows, 64))):
+        with pytest.raises(ValueError):
+            fused._norm_rows(x, res, w, out, 64)
