@@ -81,7 +81,8 @@ def add_rmsnorm_quant(x: torch.Tensor, residual: torch.Tensor | None, w: torch.T
     (E4M3, the rounding of quant_fp8_e8m0) or "fp4" (E2M1, quant_fp4), with no rounding in between.
     x, residual [..., K], w [K]: bf16, fp16 or fp32, all of one dtype; K % 32 == 0, K <= 32768. Returns (codes uint8 [..., K] or [..., K / 2],
     E8M0 bytes uint8 [..., K / 32], r), the first two being the operand of w4.linear_fp4 (FP8: of the expert GEMMs too); with `y` also
-    v rounded to x's dtype (a router's input). `out` receives r: a tensor like x, which may be x or residual itself.
+    v rounded to x's dtype (a router's input). `out` receives r: a tensor like x, which may be x or residual itself; its version counter moves
+    as with torch's own in-place operations.
     A group with a NaN or an infinity in it gets the byte 255 and codes 0x7F (FP8) or 0 (FP4), NaN in every product; a row whose mean
     square is NaN or overflows fp32 is such a row or rounds to zeros, as the formula has it.
     Inference only: inputs that need a gradient are refused."""
@@ -105,7 +106,7 @@ def add_rmsnorm_quant(x: torch.Tensor, residual: torch.Tensor | None, w: torch.T
     dev = x.device
     if not x.is_cuda or w.device != dev or (residual is not None and residual.device != dev) or (out is not None and out.device != dev):
         _lib.require_cuda(x, residual, w, out)
-    lead, rows = shape[:-1], x.numel() // K
+    lead, rows, given = shape[:-1], x.numel() // K, out is not None
     px, pw, pr, po, sx, sr, so = x.data_ptr(), w.data_ptr(), None, None, K, K, K
     if residual is not None and out is None and x.is_contiguous() and residual.is_contiguous() and w.is_contiguous() and not (
             (px | pw | (pr := residual.data_ptr())) & 15):
@@ -119,6 +120,8 @@ def add_rmsnorm_quant(x: torch.Tensor, residual: torch.Tensor | None, w: torch.T
     if rows:
         _lib.launch(dev, "dsv41_add_rmsnorm_mx", px, sx, pr, sr, pw, eps, _TYPE[dt], rows, K, bits, po, so, yt.data_ptr() if y else None,
                     codes.data_ptr(), scales.data_ptr())
+        if given:
+            torch.autograd.graph.increment_version(out)   # the launch wrote past torch: autograd and an FP8 record on out have to see it
     r = x if residual is None else out
     return (codes, scales, r, yt) if y else (codes, scales, r)
 

@@ -139,8 +139,8 @@ def attach_codes(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, per
     bf16 values from them). `permuted`: x holds the values in the 8-k permuted order of permute_x. The record is
     tied to x's version counter, storage address, shape and strides, so an in-place change of x (through x or any view
     of it), a resize or a set_ drops it; views and copies of x carry none. Library entry points that write into a
-    caller's tensor (`out=` arguments) bump no version counter: a tensor passed there must not be read as an operand
-    afterwards on the strength of an earlier record. Inference-mode tensors keep no version counter, so they get no record (an in-place change could
+    caller's tensor (`out=` arguments) bump no version counter, except add_rmsnorm_quant: a tensor passed to the others must not be
+    read as an operand afterwards on the strength of an earlier record. Inference-mode tensors keep no version counter, so they get no record (an in-place change could
     not be seen) and are quantised again where used. Returns x."""
     assert codes.shape == x.shape and scales.shape == (*x.shape[:-1], x.shape[-1] // 32)
     if not x.is_inference():

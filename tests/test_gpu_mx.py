@@ -684,3 +684,19 @@ def test_add_rmsnorm_quant_refuses_the_weight_as_output():
         fused.add_rmsnorm_quant(x, res, w, 1e-6, out=w.view(1, 5120))
     assert torch.equal(w, keep)
     assert all(torch.equal(a, b) for a, b in zip(want, fused.add_rmsnorm_quant(x, res, w, 1e-6, out=x)))
+
+
+def test_add_rmsnorm_quant_output_drops_an_fp8_record():
+    """swiglu_quant's result carries its FP8 codes; a norm that writes r over it drops them, so that a product of r is r's."""
+    from dsv41_amd import fused, quant, w4, w8
+    g = gen(42)
+    W = w4.W4(*[t.cuda() for t in rand_w4(g, 96, 256)])
+    res, n = randn(g, 9, 256, dtype=torch.bfloat16).cuda(), randn(g, 256, dtype=torch.bfloat16).cuda()
+    h = fused.swiglu_quant(randn(g, 9, 512).cuda(), None, 256, 10.0)
+    old = w4.linear_fp4(h, W, act="fp8")
+    assert quant.attached_codes(h, False) is not None
+    want = fused.add_rmsnorm_quant(h.clone(), res, n, 1e-6)
+    got = fused.add_rmsnorm_quant(h, res, n, 1e-6, out=h)
+    assert got[2] is h and all(torch.equal(a, b) for a, b in zip(want, got)) and quant.attached_codes(h, False) is None
+    y = w4.linear_fp4(want[2], W, act="fp8")
+    assert torch.equal(w4.linear_fp4(h, W, act="fp8"), y) and torch.equal(w8.linear_w(h, W), y) and not torch.equal(y, old)

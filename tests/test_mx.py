@@ -197,3 +197,36 @@ def test_norm_output_is_never_the_weight(rows):
     for w, out in ((w, w.view(1, 64).expand(rows, 64)), (buf[:64], buf[:rows * 64].view(rows, 64)), (buf[32:96], buf[:rows * 64].view(rows, 64))):
         with pytest.raises(ValueError):
             fused._norm_rows(x, res, w, out, 64)
+
+
+def test_norm_output_counts_as_changed(monkeypatch):
+    """`out` is written past torch: its version counter moves, so an FP8 record on it (or on a tensor that it is a view of) is dropped and
+    autograd sees the change. Inputs and outputs of the call's own stay as they are."""
+    from dsv41_amd import _lib, fused, quant
+    monkeypatch.setattr(_lib, "require_cuda", lambda *t: None)
+    monkeypatch.setattr(_lib, "launch", lambda *a: None)
+    recorded = lambda *s: quant.attach_codes(torch.zeros(*s, dtype=torch.bfloat16), torch.zeros(*s, dtype=torch.uint8),
+                                             torch.zeros(*s[:-1], s[-1] // 32, dtype=torch.uint8))
+    w = torch.ones(64, dtype=torch.bfloat16)
+    for pick in (lambda x, r: x, lambda x, r: r, lambda x, r: x.view(4, 64), lambda x, r: recorded(4, 64)):
+        x, res = recorded(4, 64), recorded(4, 64)
+        out = pick(x, res)
+        base = x if out._base is x else out
+        before = {id(t): t._version for t in (x, res, w)}
+        assert fused.add_rmsnorm_quant(x, res, w, 1e-6, out=out)[2] is out
+        assert quant.attached_codes(base, False) is None
+        for t in (x, res, w):
+            assert t is base or t._version == before[id(t)] and (t is w or quant.attached_codes(t, False) is not None)
+    x, res = recorded(4, 64), recorded(4, 64)
+    fused.add_rmsnorm_quant(x, res, w, 1e-6)
+    assert quant.attached_codes(x, False) is not None and quant.attached_codes(res, False) is not None
+    a = torch.ones(4, 64, dtype=torch.bfloat16, requires_grad=True)
+    h = a * 2
+    loss = (h * h).sum()
+    with torch.no_grad():
+        fused.add_rmsnorm_quant(torch.zeros_like(h), h, w, 1e-6, out=h)
+    with pytest.raises(RuntimeError, match="inplace operation"):
+        loss.backward()
+    with torch.inference_mode():
+        h = torch.zeros(4, 64, dtype=torch.bfloat16)
+        assert fused.add_rmsnorm_quant(h, h, w, 1e-6, out=h)[2] is h
