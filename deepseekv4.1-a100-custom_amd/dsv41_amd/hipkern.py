@@ -436,7 +436,7 @@ MX_ROWS = 16       # rows that the kernel for few rows takes
 
 
 def _mx_chunk(nk: int) -> int:
-    """Rows of one launch: the tile kernels' scale array has 32-bit offsets, their quantiser a grid of rows."""
+    """Rows of one launch: the tile kernels' scale array has 32-bit offsets, their quantiser a grid of rows. 65535 at least (K = 2^20)."""
     return min(1 << 19, ((1 << 29) - 1) // nk)
 
 
@@ -491,7 +491,7 @@ def mx_linear(x2: torch.Tensor, fmt: int, w, dtype: torch.dtype) -> torch.Tensor
     M = x2.shape[0]
     dev = x2.device
     y = torch.empty((M, N), dtype=dtype, device=dev)
-    if M > 1 << 16 and M > (n := _mx_chunk(-(-K // 128))):
+    if M >= 1 << 16 and M > (n := _mx_chunk(-(-K // 128))):
         for i in range(0, M, n):
             y[i:i + n] = mx_linear(x2[i:i + n], fmt, w, dtype)
     elif M:
@@ -509,7 +509,7 @@ def mx_gemm(codes: torch.Tensor, scales: torch.Tensor, fmt: int, w, dtype: torch
     M = codes.shape[0]
     dev = codes.device
     y = torch.empty((M, N), dtype=dtype, device=dev)
-    if M > 1 << 16 and M > (n := _mx_chunk(-(-K // 128))):
+    if M >= 1 << 16 and M > (n := _mx_chunk(-(-K // 128))):
         for i in range(0, M, n):
             y[i:i + n] = mx_gemm(codes[i:i + n], scales[i:i + n], fmt, w, dtype)
     elif M:

@@ -230,3 +230,24 @@ def test_norm_output_counts_as_changed(monkeypatch):
     with torch.inference_mode():
         h = torch.zeros(4, 64, dtype=torch.bfloat16)
         assert fused.add_rmsnorm_quant(h, h, w, 1e-6, out=h)[2] is h
+
+
+@pytest.mark.parametrize("K", [32, 128, 1024, 131072, (1 << 20) - 32, 1 << 20])
+def test_rows_of_a_launch_fit_its_offsets(monkeypatch, K):
+    """Every launch of mx_linear and mx_gemm has rows x tiles of 128 k below 2^29 and at most 65535 x 16 rows, at row counts around the
+    limits; the launches together are all rows, once."""
+    from dsv41_amd import _lib, hipkern
+    seen = []
+    monkeypatch.setattr(_lib, "launch", lambda dev, name, *a: seen.append((name, a[3], a[8] if name.endswith("linear") else a[9])))
+    nk = -(-K // 128)
+    limit = min(65535 * 16, ((1 << 29) - 1) // nk)
+
+    class W:
+        shape, w4, s4 = (1, K), torch.empty(0), torch.empty(0)
+    for M in sorted({1, 17, 65535, 65536, 65537, limit, limit + 1, 2 * limit + 3}):
+        for call in (lambda: hipkern.mx_linear(torch.empty(M, K, dtype=torch.bfloat16, device="meta"), 8, W, torch.bfloat16),
+                     lambda: hipkern.mx_gemm(torch.empty(M, K, dtype=torch.uint8, device="meta"), torch.empty(M, K // 32, dtype=torch.uint8, device="meta"),
+                                             8, W, torch.bfloat16)):
+            seen.clear()
+            assert call().shape == (M, 1)
+            assert sum(rows for _, _, rows in seen) == M and all(k == K and 0 < rows <= limit for _, k, rows in seen), (M, seen)
