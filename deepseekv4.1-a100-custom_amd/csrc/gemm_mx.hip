@@ -436,14 +436,16 @@ static int allow_lds(const void* kernel, int bytes, std::atomic<uint64_t>& known
     return 0;
 }
 
+// `launch` false: only whether the launch can be made
 template <int AF, int WM, int WT, int NT, int KP, int NS>
-static int launch_tiles(const MxArgs& a, hipStream_t st) {
+static int launch_tiles(const MxArgs& a, bool launch, hipStream_t st) {
     using C = Tile<AF, WM, WT, NT, KP, NS>;
     static_assert(C::LDS <= 160 * 1024, "LDS of one CU");
     static std::atomic<uint64_t> known{0};
-    if (const int e = allow_lds((const void*)&mx_gemm_kernel<AF, WM, WT, NT, KP, NS>, C::LDS, known)) return e;
     const long long tiles = ((long long)((a.N + C::BW - 1) / C::BW) * ((a.M + C::BT - 1) / C::BT) * a.split + 7) / 8 * 8;
     if (tiles > 0xFFFFFFFFll / C::THREADS) return DSV41_EINVAL;   // a launch holds fewer than 2^32 threads
+    if (!launch) return 0;
+    if (const int e = allow_lds((const void*)&mx_gemm_kernel<AF, WM, WT, NT, KP, NS>, C::LDS, known)) return e;
     mx_gemm_kernel<AF, WM, WT, NT, KP, NS><<<(unsigned)tiles, C::THREADS, C::LDS, st>>>(a);
     return (int)hipGetLastError();
 }
@@ -680,18 +682,19 @@ static bool mx_bad_weights(const uint8_t* w, const uint8_t* s, int N, int K, con
            ((((uintptr_t)w) | ((uintptr_t)s) | ((uintptr_t)y)) & 15);
 }
 
-// The tile kernels, on scales [K / 128][M][4] (32-bit offsets into them)
-static int mx_tiles(const MxArgs& a, int fmt, int plan, hipStream_t st) {
+// The tile kernels, on scales [K / 128][M][4] (32-bit offsets into them); `launch` false: only whether they take the call, which is asked
+// before the operand is made
+static int mx_tiles(const MxArgs& a, int fmt, int plan, bool launch, hipStream_t st) {
     plan &= 15;
     if ((long long)a.M * a.nk > (1ll << 29) - 1) return DSV41_EINVAL;
     if (fmt == 4) {
-        if (plan == 0) return launch_tiles<4, 1, 1, 2, 2, 4>(a, st);
-        if (plan == 1) return launch_tiles<4, 2, 2, 2, 1, 4>(a, st);
-        if (plan == 2) return launch_tiles<4, 4, 2, 4, 2, 2>(a, st);
+        if (plan == 0) return launch_tiles<4, 1, 1, 2, 2, 4>(a, launch, st);
+        if (plan == 1) return launch_tiles<4, 2, 2, 2, 1, 4>(a, launch, st);
+        if (plan == 2) return launch_tiles<4, 4, 2, 4, 2, 2>(a, launch, st);
     } else {
-        if (plan == 0) return launch_tiles<0, 1, 1, 2, 2, 3>(a, st);
-        if (plan == 1) return launch_tiles<0, 2, 2, 2, 1, 3>(a, st);
-        if (plan == 2) return launch_tiles<0, 4, 2, 4, 1, 3>(a, st);
+        if (plan == 0) return launch_tiles<0, 1, 1, 2, 2, 3>(a, launch, st);
+        if (plan == 1) return launch_tiles<0, 2, 2, 2, 1, 3>(a, launch, st);
+        if (plan == 2) return launch_tiles<0, 4, 2, 4, 1, 3>(a, launch, st);
     }
     return DSV41_EINVAL;
 }
@@ -712,8 +715,10 @@ extern "C" int dsv41_mx_gemm(const uint8_t* w, const uint8_t* s, int N, int K, c
     const MxParts parts(plan, N, M, 4ll * M * nk);
     if (!ws || (((uintptr_t)ws) & 15) || ws_bytes < parts.end) return DSV41_EINVAL;
     uint32_t* const count = (uint32_t*)(ws + parts.count);
+    const MxArgs a{w, s, N, nk, xc, ldx, K / 8 * fmt, ws, M, y, ldy, out_type, parts.n, count, (float*)(ws + parts.part)};
+    if (const int e = mx_tiles(a, fmt, plan, false, st)) return e;
     if (const int e = mx_turn_scales(xs, ldxs, M, K, ws, count, parts.counters, st)) return e;
-    return mx_tiles(MxArgs{w, s, N, nk, xc, ldx, K / 8 * fmt, ws, M, y, ldy, out_type, parts.n, count, (float*)(ws + parts.part)}, fmt, plan, st);
+    return mx_tiles(a, fmt, plan, true, st);
 }
 
 extern "C" int dsv41_mx_linear(const uint8_t* w, const uint8_t* s, int N, int K, const void* x, int dtype, long long ldx, int fmt, int M, int out_type,
@@ -736,6 +741,8 @@ extern "C" int dsv41_mx_linear(const uint8_t* w, const uint8_t* s, int N, int K,
     const MxParts parts(plan, N, M, M * (row + nk * 4));
     if (!ws || (((uintptr_t)ws) & 15) || ws_bytes < parts.end) return DSV41_EINVAL;
     uint32_t* const count = (uint32_t*)(ws + parts.count);
+    const MxArgs a{w, s, N, nk, ws, row, (int)row, ws + M * row, M, y, ldy, out_type, parts.n, count, (float*)(ws + parts.part)};
+    if (const int e = mx_tiles(a, fmt, plan, false, st)) return e;
     if (const int e = mx_quant_operand(x, dtype, M, K, ldx, fmt, nk, ws, ws + M * row, count, parts.counters, st)) return e;
-    return mx_tiles(MxArgs{w, s, N, nk, ws, row, (int)row, ws + M * row, M, y, ldy, out_type, parts.n, count, (float*)(ws + parts.part)}, fmt, plan, st);
+    return mx_tiles(a, fmt, plan, true, st);
 }

@@ -251,3 +251,29 @@ def test_rows_of_a_launch_fit_its_offsets(monkeypatch, K):
             seen.clear()
             assert call().shape == (M, 1)
             assert sum(rows for _, _, rows in seen) == M and all(k == K and 0 < rows <= limit for _, k, rows in seen), (M, seen)
+
+
+def test_c_entries_refuse_before_the_operand():
+    """Sizes that the product's launch cannot take are refused before the launch that makes its operand. Addresses are never read: a call that
+    is let through ends with the runtime's error where there is no GPU, and is not made where there is one."""
+    from dsv41_amd import _lib
+    if not os.path.exists(_lib.LIB_PATH):
+        pytest.skip("library not built")
+    if torch.cuda.is_available():
+        pytest.skip("a call that is not refused would launch")
+    L = _lib.lib()
+    p, big = ctypes.c_void_p(4096), (1 << 62)
+
+    def gemm(N=64, K=256, fmt=8, M=64, plan=0):
+        return L.dsv41_mx_gemm(p, p, N, K, p, K * fmt // 8, p, K // 32, fmt, M, 0, p, N, plan, p, big, None)
+
+    def linear(N=64, K=256, fmt=8, M=64, plan=0):
+        return L.dsv41_mx_linear(p, p, N, K, p, 0, K, fmt, M, 0, p, N, plan, p, big, None)
+    for call in (gemm, linear):
+        assert call() > 0                                         # no device
+        for fmt in (4, 8):
+            for plan in (0, 1, 2):
+                assert call(fmt=fmt, plan=plan, M=65536, K=1 << 20) == -1            # rows x tiles of 128 k: 2^29
+                assert call(fmt=fmt, plan=plan, M=65535, K=1 << 20) > 0
+                assert call(fmt=fmt, plan=plan, M=1 << 19, N=1 << 29, K=32) == -1    # tiles
+    assert linear(M=1048561, K=32) == -1 and linear(M=1048560, K=32) > 0             # rows of the rounding's launch
