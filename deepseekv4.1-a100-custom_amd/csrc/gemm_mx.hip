@@ -638,9 +638,11 @@ __global__ void __launch_bounds__((SK_STREAM + SK_QUANT) * 64, 8) mx_rows_kernel
 template <int AF, int XT, int RB>
 static int launch_rows_v(const MxRowsArgs& a, hipStream_t st) {
     static std::atomic<uint64_t> known{0};
+    constexpr int threads = (SK_STREAM + SK_QUANT) * 64;
+    const int blocks = ((a.N + 15) / 16 + RB - 1) / RB;
+    if (blocks > 0xFFFFFFFFll / threads) return DSV41_EINVAL;   // a launch holds fewer than 2^32 threads: N < 2^29
     if (const int e = allow_lds((const void*)&mx_rows_kernel<AF, XT, RB>, 160 * 1024, known)) return e;
-    const int tiles = (a.N + 15) / 16;
-    mx_rows_kernel<AF, XT, RB><<<(unsigned)((tiles + RB - 1) / RB), (SK_STREAM + SK_QUANT) * 64, sk_lds<AF>(a.M, a.nk), st>>>(a);
+    mx_rows_kernel<AF, XT, RB><<<(unsigned)blocks, threads, sk_lds<AF>(a.M, a.nk), st>>>(a);
     return (int)hipGetLastError();
 }
 
@@ -678,7 +680,7 @@ struct MxParts {
 };
 
 static bool mx_bad_weights(const uint8_t* w, const uint8_t* s, int N, int K, const void* y, long long ldy, int out_type) {
-    return !w || !s || !y || N < 1 || K < 32 || (K & 31) || K > (1 << 20) || out_type < 0 || out_type > 2 || ldy < N ||
+    return !w || !s || !y || N < 1 || N > (1 << 30) || K < 32 || (K & 31) || K > (1 << 20) || out_type < 0 || out_type > 2 || ldy < N ||
            ((((uintptr_t)w) | ((uintptr_t)s) | ((uintptr_t)y)) & 15);
 }
 

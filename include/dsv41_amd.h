@@ -391,7 +391,8 @@ int dsv41_add_rmsnorm_mx(const void* x, long long ldx, const void* res, long lon
  * ldx % 16 == 0. plan: tiles of 64 x 64 (0, weight rows x tokens), 128 x 128 (1) or 256 x 256 (2), which bring the scales
  * into their own order first, in ws (16-byte aligned, ws_bytes >= 4 M ceil(K / 128)); or 3, the kernel for at most 16 rows, which needs
  * M (nk (32 fmt + 8) + 20) + 15 + 8192 <= 160 KiB of LDS, nk = ceil(K / 256), and no workspace. Plan 0 + 16 p, 2 <= p <= ceil(K / 256):
- * K in p parts whose sums are added in their order, for few tiles of a long K; ws then has 16 + ceil(N / 64) ceil(M / 64) (16 + 16384 p) bytes more. Tiles: M <= 1048560, M K / 128 < 2^29. */
+ * K in p parts whose sums are added in their order, for few tiles of a long K; ws then has 16 + ceil(N / 64) ceil(M / 64) (16 + 16384 p) bytes more.
+ * K <= 2^20. Tiles: M <= 1048560, M ceil(K / 128) < 2^29, fewer than 2^23 tiles (times p). Plan 3: N < 2^29. */
 int dsv41_mx_gemm(const uint8_t* w, const uint8_t* s, int N, int K, const uint8_t* xc, long long ldx, const uint8_t* xs, long long ldxs, int fmt,
                   int M, int out_type, void* y, long long ldy, int plan, uint8_t* ws, long long ws_bytes, void* stream);
 

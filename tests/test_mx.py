@@ -277,3 +277,27 @@ def test_c_entries_refuse_before_the_operand():
                 assert call(fmt=fmt, plan=plan, M=65535, K=1 << 20) > 0
                 assert call(fmt=fmt, plan=plan, M=1 << 19, N=1 << 29, K=32) == -1    # tiles
     assert linear(M=1048561, K=32) == -1 and linear(M=1048560, K=32) > 0             # rows of the rounding's launch
+
+
+def test_c_entries_refuse_more_weight_rows_than_a_launch_holds():
+    """2^29 weight rows: the kernel for few rows would need 2^32 threads, and row counts next to 2^31 would wrap while tiles are counted."""
+    from dsv41_amd import _lib
+    if not os.path.exists(_lib.LIB_PATH):
+        pytest.skip("library not built")
+    if torch.cuda.is_available():
+        pytest.skip("a call that is not refused would launch")
+    L = _lib.lib()
+    p, big = ctypes.c_void_p(4096), (1 << 62)
+
+    def gemm(N, fmt, plan):
+        return L.dsv41_mx_gemm(p, p, N, 32, p, 2 * fmt * 4, p, 1, fmt, 1, 0, p, N, plan, p, big, None)
+
+    def linear(N, fmt, plan):
+        return L.dsv41_mx_linear(p, p, N, 32, p, 0, 32, fmt, 1, 0, p, N, plan, p, big, None)
+    for call in (gemm, linear):
+        for fmt in (4, 8):
+            assert call((1 << 29) - 128, fmt, 3) > 0              # no device
+            assert call(1 << 29, fmt, 3) == -1
+            for plan in (0, 1, 2, 3):
+                assert call((1 << 31) - 1, fmt, plan) == -1
+                assert call((1 << 31) - 64, fmt, plan) == -1
