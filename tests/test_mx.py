@@ -301,3 +301,16 @@ def test_c_entries_refuse_more_weight_rows_than_a_launch_holds():
             for plan in (0, 1, 2, 3):
                 assert call((1 << 31) - 1, fmt, plan) == -1
                 assert call((1 << 31) - 64, fmt, plan) == -1
+
+
+def test_quant_fp4_refuses_a_gradient():
+    """Its values would take x's place without a graph. Without grad mode, and for detached weights, there is nothing to lose."""
+    from dsv41_amd import quant, w4
+    x = torch.zeros(4, 64, requires_grad=True)
+    for values in (False, True):
+        with pytest.raises(RuntimeError, match="gradient"):
+            quant.quant_fp4(x, values=values)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="GPU only"):
+            quant.quant_fp4(x, values=values)
+    with pytest.raises(RuntimeError, match="GPU only"):
+        w4.W4.from_dense(x)
