@@ -314,3 +314,13 @@ def test_quant_fp4_refuses_a_gradient():
             quant.quant_fp4(x, values=values)
     with pytest.raises(RuntimeError, match="GPU only"):
         w4.W4.from_dense(x)
+
+
+def test_norm_refuses_an_output_that_needs_a_gradient():
+    from dsv41_amd import fused
+    x, w = torch.zeros(4, 64), torch.ones(64)
+    for out in (torch.zeros(4, 64, requires_grad=True), torch.zeros(4, 64, requires_grad=True) * 1):
+        with pytest.raises(RuntimeError, match="gradient"):
+            fused.add_rmsnorm_quant(x, x, w, 1e-6, out=out)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="GPU only"):
+            fused.add_rmsnorm_quant(x, x, w, 1e-6, out=out)
