@@ -14,6 +14,7 @@ import ctypes
 import os
 
 import torch
+from torch.autograd import forward_ad
 
 _PKG_ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 LIB_PATH = os.environ.get("DSV41_AMD_LIB", os.path.join(_PKG_ROOT, "lib", "libdsv41_amd.so"))
@@ -121,6 +122,24 @@ def launch(dev: torch.device, name: str, *args) -> None:
     err = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     if err:
         check(err, name)
+
+
+_grad_enabled, _tracing, _modes, _mode = torch.is_grad_enabled, torch._C._is_tracing, torch._C._len_torch_dispatch_stack, torch._C._get_dispatch_mode
+_PROXY = torch._C._TorchDispatchModeKey.PROXY
+
+
+def inference_only(what: str, *ts: torch.Tensor | None) -> None:
+    """Refuses a call in which torch follows more than the values, which a direct launch would pass by: reverse or forward mode
+    gradients of ts (None is skipped), and tracers (jit.trace, make_fx), which would record the empty outputs alone."""
+    for t in ts:
+        if t is not None and t.requires_grad and _grad_enabled():
+            raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad() or detach its tensors")
+    if forward_ad._current_level >= 0:
+        for t in ts:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{what} has no forward-mode gradient: give it the primal values")
+    if _tracing() or (_modes() and _mode(_PROXY) is not None):
+        raise RuntimeError(f"{what} cannot be traced: a trace would hold its outputs without the launch that fills them")
 
 
 def row_stride(t: torch.Tensor) -> int:

@@ -85,7 +85,7 @@ def add_rmsnorm_quant(x: torch.Tensor, residual: torch.Tensor | None, w: torch.T
     as with torch's own in-place operations.
     A group with a NaN or an infinity in it gets the byte 255 and codes 0x7F (FP8) or 0 (FP4), NaN in every product; a row whose mean
     square is NaN or overflows fp32 is such a row or rounds to zeros, as the formula has it.
-    Inference only: inputs (and an out) that need a gradient are refused."""
+    Inference only: inputs (and an out) with a gradient to follow (reverse or forward mode) are refused, and so is a tracer."""
     bits, dt, shape = _BITS.get(fmt), x.dtype, x.shape
     if bits is None:
         raise ValueError(f"fmt is 'fp8' or 'fp4', got {fmt!r}")
@@ -101,9 +101,7 @@ def add_rmsnorm_quant(x: torch.Tensor, residual: torch.Tensor | None, w: torch.T
         raise ValueError(f"residual and out are shaped like x {tuple(shape)}, got {[tuple(t.shape) for t in (residual, out) if t is not None]}")
     if out is not None and residual is None:
         raise ValueError("without a residual r is x itself: there is nothing to write into out")
-    if (x.requires_grad or w.requires_grad or (residual is not None and residual.requires_grad) or (
-            out is not None and out.requires_grad)) and torch.is_grad_enabled():
-        raise RuntimeError("add_rmsnorm_quant has no gradient: call it under torch.no_grad() or detach its inputs and out")
+    _lib.inference_only("add_rmsnorm_quant", x, residual, w, out)
     dev = x.device
     if not x.is_cuda or w.device != dev or (residual is not None and residual.device != dev) or (out is not None and out.device != dev):
         _lib.require_cuda(x, residual, w, out)

@@ -64,7 +64,7 @@ def quant_fp4(x: torch.Tensor, block: int = 32, values: bool = False):
     `values`: also the bf16 values that the codes stand for (dequant_fp4 of the two), from the same launch; an amax above 1.75 * 2^127
     rounds up to 2^128, infinity in bf16.
     A group with a NaN or an infinity in it gets the byte 255 and zero codes: dequant_fp4 and the product give NaN for all of it.
-    Inference only: an x that needs a gradient is refused."""
+    Inference only: an x with a gradient to follow (reverse or forward mode) is refused, and so is a tracer."""
     if block != 32:
         raise ValueError(f"quant_fp4 has groups of 32, got {block}")
     dt, shape = x.dtype, x.shape
@@ -73,8 +73,7 @@ def quant_fp4(x: torch.Tensor, block: int = 32, values: bool = False):
     K = shape[-1] if shape else 0
     if K % 32 or K == 0:
         raise ValueError(f"quant_fp4: the last dimension is a multiple of 32, got {tuple(shape)}")
-    if x.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError("quant_fp4 has no gradient: call it under torch.no_grad() or detach x")
+    _lib.inference_only("quant_fp4", x)
     if not x.is_cuda:
         _lib.require_cuda(x)
     dev, lead, rows, ld = x.device, shape[:-1], x.numel() // K, K

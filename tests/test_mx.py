@@ -324,3 +324,42 @@ def test_norm_refuses_an_output_that_needs_a_gradient():
             fused.add_rmsnorm_quant(x, x, w, 1e-6, out=out)
         with torch.no_grad(), pytest.raises(RuntimeError, match="GPU only"):
             fused.add_rmsnorm_quant(x, x, w, 1e-6, out=out)
+
+
+def _entries():
+    """The three entry points as functions of one float matrix [4, 64]."""
+    from dsv41_amd import fused, quant, w4, w8
+    W, n = w4.W4(*rand_w4(20, 64)), torch.ones(64)
+    pair = torch.zeros(4, 64, dtype=torch.uint8), torch.zeros(4, 2, dtype=torch.uint8)
+    return {"quant_fp4": lambda x: quant.quant_fp4(x, values=True)[2], "linear_fp4": lambda x: w4.linear_fp4(x, W), "linear_w": lambda x: w8.linear_w(x, W),
+            "pair": lambda x: w4.linear_fp4(pair, W) + x[:, :20], "norm": lambda x: fused.add_rmsnorm_quant(x, x, n, 1e-6)[2],
+            "norm residual": lambda x: fused.add_rmsnorm_quant(torch.zeros(4, 64), x, n, 1e-6)[2],
+            "norm weight": lambda x: fused.add_rmsnorm_quant(torch.zeros(4, 64), None, x[0], 1e-6, y=True)[3],
+            "norm out": lambda x: fused.add_rmsnorm_quant(torch.zeros(4, 64), torch.zeros(4, 64), n, 1e-6, out=x)[2]}
+
+
+@pytest.mark.parametrize("name", ["quant_fp4", "linear_fp4", "linear_w", "norm", "norm residual", "norm weight", "norm out"])
+def test_forward_mode_tangents_are_refused(name):
+    """A launch would drop an input's tangent; without one, a dual level around the call is nothing to it."""
+    import torch.autograd.forward_ad as fwd
+    call = _entries()[name]
+    with fwd.dual_level():
+        x = fwd.make_dual(torch.zeros(4, 64), torch.ones(4, 64))
+        with pytest.raises(RuntimeError, match="gradient"):
+            call(x)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="gradient"):
+            call(x)
+        with torch.inference_mode(), pytest.raises(RuntimeError, match="GPU only"):
+            call(x)
+        with pytest.raises(RuntimeError, match="GPU only"):
+            call(torch.zeros(4, 64))
+
+
+@pytest.mark.parametrize("name", ["quant_fp4", "linear_fp4", "linear_w", "pair", "norm"])
+def test_traces_are_refused(name):
+    """torch's tracers would record the empty outputs and not the launch."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    call = _entries()[name]
+    for trace in (lambda: torch.jit.trace(call, torch.zeros(4, 64)), lambda: make_fx(call)(torch.zeros(4, 64))):
+        with pytest.raises(RuntimeError, match="trace"):
+            trace()
