@@ -23,6 +23,7 @@ import torch
 
 from . import _lib
 from .fused2 import _MODES
+from .w4 import W4
 
 
 @dataclass
@@ -81,12 +82,19 @@ class SharedExpert:
     def fp8(self) -> bool:
         return self.s13 is not None
 
+    @staticmethod
+    def _no_w4(w13, w2):
+        if isinstance(w13, W4) or isinstance(w2, W4):
+            raise TypeError("the decode launches read no W4 shared expert: give the pair to moe_experts, moe_route_experts, MoE or OffloadMoE")
+
     @classmethod
     def of(cls, shared) -> "SharedExpert | None":
-        """A SharedExpert from one, from a (w13, w2) row-major bf16 pair, or from a (W8, W8) pair; None stays None."""
+        """A SharedExpert from one, from a (w13, w2) row-major bf16 pair, or from a (W8, W8) pair; None stays None. FP4 pairs are none
+        (shared_expert_rows computes them)."""
         if shared is None or isinstance(shared, SharedExpert):
             return shared
         w13, w2 = shared
+        cls._no_w4(w13, w2)
         from .w8 import W8
         if isinstance(w13, W8):
             return cls.prepare_w8(w13, w2)
@@ -96,6 +104,7 @@ class SharedExpert:
     def prepare(cls, w13: torch.Tensor, w2: torch.Tensor, tiled: bool = True) -> "SharedExpert":
         """From row-major [w1; w3] and w2 (bf16, on the GPU), repacked once into the tiled layout when `tiled`."""
         from .quant import tile_bf16
+        cls._no_w4(w13, w2)
         w13, w2 = w13.to(torch.bfloat16).contiguous(), w2.to(torch.bfloat16).contiguous()
         return cls(tile_bf16(w13), tile_bf16(w2), True) if tiled else cls(w13, w2, False)
 
@@ -265,19 +274,17 @@ def decode_down(ws: _Workspace, ex: ExpertWeights, ys=None, out=None, y32=None, 
 
 
 def _shared_plan(xq, shared, ys, k, ex, limit, ys_out):
-    """(shared expert for the fused launches or None, ys): the bf16 shared expert rides in the two decode launches when
-    it fits them; otherwise it runs first as its own launches and enters as ys."""
-    from .w4 import W4
-    four = isinstance(shared, (tuple, list)) and isinstance(shared[0], W4)
-    sh = None if four else SharedExpert.of(shared)
-    if sh is None and not four:
+    """(shared expert for the fused launches or None, ys): the bf16 or FP8 shared expert rides in the two decode launches when
+    it fits them; otherwise, and with FP4 weights (a pair of w4.W4), it runs first as its own launches and enters as ys."""
+    if shared is None:
         return None, ys
     assert ys is None, "give either the shared expert's weights or its output"
-    if four:   # FP4 weights: launches of their own
+    if isinstance(shared, (tuple, list)) and isinstance(shared[0], W4):
         y_s = shared_expert_rows(xq, *shared, ex.I, limit)
         if ys_out is not None:
             ys_out.copy_(y_s)
         return None, y_s
+    sh = SharedExpert.of(shared)
     if fused_shared_ok(xq.shape[0], k, ex.I, sh.fp8):
         return sh, None
     if sh.fp8:
@@ -299,9 +306,9 @@ def moe_experts(xq: torch.Tensor, eid: torch.Tensor, wt: torch.Tensor, ex: Exper
     PAIRS_MAX_M, which runs pair by pair); wt fp32 [M, k].
     Returns fp32 [M, H] = sum_j w_j-weighted expert outputs (routing weight folded into h, fused.py:297-302),
     or, when `out` (bf16 [M, H]) is given, writes out = bf16(y + ys) (ys: bf16 shared-expert output or None);
-    y32 (fp32 [M, H]) additionally receives y. shared (a SharedExpert, or a row-major (w13, w2) bf16 pair) computes
-    the shared expert too (model.py:409-412) instead of taking ys: in the same two launches when it fits them
-    (fused_shared_ok), else as its own launches first; ys_out (bf16 [M, H]) receives its output. hc = (residual, post,
+    y32 (fp32 [M, H]) additionally receives y. shared (a SharedExpert, a row-major (w13, w2) bf16 pair, or a pair of w8.W8 or
+    w4.W4) computes the shared expert too (model.py:409-412) instead of taking ys: in the same two launches when it fits them
+    (fused_shared_ok; never W4), else as its own launches first; ys_out (bf16 [M, H]) receives its output. hc = (residual, post,
     comb) applies the hyper-connection post mix to bf16(y + ys) in the same launch (decode_down)."""
     k = eid.shape[-1]
     M = xq.shape[0]
@@ -616,7 +623,6 @@ class MoE:
         self.gate_w = gate_w.to(torch.float32).contiguous()                       # fp32 [E, dim] (model.py:368)
         assert self.gate_w.shape == (self.n_experts, self.dim)
         self.gate_bias = None if gate_bias is None else gate_bias.to(torch.float32).contiguous()
-        from .w4 import W4
         from .w8 import W8
         self.shared = None
         if isinstance(sh_w13, W4):

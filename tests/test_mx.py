@@ -363,3 +363,17 @@ def test_traces_are_refused(name):
     for trace in (lambda: torch.jit.trace(call, torch.zeros(4, 64)), lambda: make_fx(call)(torch.zeros(4, 64))):
         with pytest.raises(RuntimeError, match="trace"):
             trace()
+
+
+def test_w4_pairs_are_no_shared_expert_of_the_decode_launches():
+    """The two decode launches read bf16 or FP8 shared experts; moe_experts runs an FP4 pair as launches of its own. Where the launches are
+    asked for directly, and in the layers that only know them, a W4 is named instead of failing inside."""
+    from dsv41_amd import moe, w4
+    W = w4.W4(*rand_w4(32, 64))
+    for pair in ((W, W), [W, W], (W, torch.zeros(64, 16)), (torch.zeros(32, 64), W)):
+        with pytest.raises(TypeError, match="W4"):
+            moe.SharedExpert.of(pair)
+    with pytest.raises(TypeError, match="W4"):
+        moe.SharedExpert.prepare(W, W)
+    bf = moe.SharedExpert.of((torch.zeros(32, 64), torch.zeros(64, 16)))
+    assert not bf.tiled and moe.SharedExpert.of(bf) is bf and moe.SharedExpert.of(None) is None
