@@ -167,7 +167,9 @@ def linear_fp8(x: torch.Tensor, w) -> torch.Tensor:
 def oproj_a(o: torch.Tensor, wo_a, n_groups: int, rank: int) -> torch.Tensor:
     """Grouped output projection (w8.py:116-124): o [b, s, g, d], wo_a [g * rank, d]; output columns
     g' * rank .. (g' + 1) * rank - 1 are o[..., g', :] times rows g' * rank .. of wo_a, so the result is [b, s, g * rank]
-    (a block-diagonal weight applied without materialising its zero blocks)."""
+    (a block-diagonal weight applied without materialising its zero blocks). wo_a is a bf16 tensor or a W8."""
+    if isinstance(wo_a, W4):
+        raise TypeError("oproj_a takes bf16 or W8 weights: give it a W4's bf16()")
     b, s, g, d = o.shape
     if isinstance(wo_a, W8) and b * s <= MAX_TC_ROWS and (wo_a.bf16w is None or b * s < BF16_ROWS):
         y = hipkern.fp8_gemm_tc(o.reshape(b * s * g, d).contiguous().to(torch.bfloat16), wo_a.w8, wo_a.s8, group_cols=rank,

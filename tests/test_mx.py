@@ -377,3 +377,10 @@ def test_w4_pairs_are_no_shared_expert_of_the_decode_launches():
         moe.SharedExpert.prepare(W, W)
     bf = moe.SharedExpert.of((torch.zeros(32, 64), torch.zeros(64, 16)))
     assert not bf.tiled and moe.SharedExpert.of(bf) is bf and moe.SharedExpert.of(None) is None
+
+
+def test_oproj_a_names_w4():
+    """The grouped output projection has no FP4 form: the dequantised weights are the caller's choice."""
+    from dsv41_amd import w4, w8
+    with pytest.raises(TypeError, match="W4"):
+        w8.oproj_a(torch.zeros(1, 2, 2, 64, dtype=torch.bfloat16), w4.W4(*rand_w4(32, 64)), 2, 16)
