@@ -25,8 +25,8 @@ class W4:
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor):
         """codes: uint8 [N, K / 2], two E2M1 codes per byte, the even k in the low nibble; scales: E8M0 bytes [N, K / 32], as quant_fp4
         and a checkpoint give them (any one-byte type, read as bytes). K % 32 == 0. Laid out once, here."""
-        if codes.element_size() != 1 or scales.element_size() != 1:
-            raise TypeError(f"W4: codes and scales are bytes, got {codes.dtype} and {scales.dtype}")
+        if scales.element_size() != 1:   # codes in wider words either hold the same bytes or do not fit the scales
+            raise TypeError(f"W4: scales are E8M0 bytes, got {scales.dtype}")
         codes, scales = codes.view(torch.uint8), scales.view(torch.uint8)
         if codes.dim() != 2 or scales.dim() != 2 or codes.shape[1] % 16 or codes.shape[1] == 0 or codes.shape[0] == 0:
             raise ValueError(f"W4: codes [N, K / 2] with K % 32 == 0 and scales [N, K / 32], got {tuple(codes.shape)} and {tuple(scales.shape)}")

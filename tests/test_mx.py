@@ -386,15 +386,20 @@ def test_oproj_a_names_w4():
         w8.oproj_a(torch.zeros(1, 2, 2, 64, dtype=torch.bfloat16), w4.W4(*rand_w4(32, 64)), 2, 16)
 
 
-def test_w4_takes_bytes_only():
-    """Wider elements would be read as several codes or scale bytes each (fp32 scales of blocks of 128 have just the bytes of E8M0's 32)."""
+def test_w4_scales_are_bytes():
+    """Wider elements would be read as several scale bytes each (fp32 scales of blocks of 128 have just the bytes of E8M0's 32); wider codes
+    either hold the same bytes or do not fit the scales."""
     from dsv41_amd import w4
     codes, scales = rand_w4(16, 256)
     for c, s in ((codes, torch.ones(16, 2)), (codes.long(), scales.long()), (codes.to(torch.bfloat16), scales.to(torch.bfloat16)),
-                 (codes.view(torch.int32), scales), (codes, scales.view(torch.int32)), (torch.zeros(16, 128), scales)):
+                 (codes, scales.view(torch.int32))):
         with pytest.raises(TypeError, match="byte"):
             w4.W4(c, s)
+    for c in (codes.long(), torch.zeros(16, 128), torch.zeros(16, 256, dtype=torch.bfloat16)):
+        with pytest.raises(ValueError):
+            w4.W4(c, scales)
     want = w4.W4(codes, scales)
-    for c, s in ((codes.view(torch.int8), scales.view(torch.float8_e8m0fnu)), (codes.view(torch.float4_e2m1fn_x2), scales), (codes, scales.view(torch.int8))):
+    for c, s in ((codes.view(torch.int8), scales.view(torch.float8_e8m0fnu)), (codes.view(torch.float4_e2m1fn_x2), scales), (codes.view(torch.int32), scales),
+                 (codes, scales.view(torch.int8))):
         W = w4.W4(c, s)
         assert torch.equal(W.w4, want.w4) and torch.equal(W.s4, want.s4)
