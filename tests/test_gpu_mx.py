@@ -700,3 +700,42 @@ def test_add_rmsnorm_quant_output_drops_an_fp8_record():
     assert got[2] is h and all(torch.equal(a, b) for a, b in zip(want, got)) and quant.attached_codes(h, False) is None
     y = w4.linear_fp4(want[2], W, act="fp8")
     assert torch.equal(w4.linear_fp4(h, W, act="fp8"), y) and torch.equal(w8.linear_w(h, W), y) and not torch.equal(y, old)
+
+
+@pytest.mark.parametrize("fmt", [4, 8])
+@pytest.mark.parametrize("dtype", DT)
+def test_c_quantiser_both_formats_and_padding(dtype, fmt):
+    """dsv41_mx_quant as a C caller has it: E2M1 and E4M3 codes of strided rows, columns K .. Kp - 1 as zero codes under a zero group's scale
+    byte, groups that are not finite marked, scale borders, and nothing written behind the last row."""
+    from dsv41_amd import _lib, quant
+    t = DT[dtype]
+    for rows, K, Kp in ((1, 32, 32), (5, 96, 128), (33, 1184, 1280), (300, 160, 160), (7, 64, 512)):
+        x = randn(gen(51 + rows), rows, K, dtype=t, spread=2.0)
+        if rows > 4:
+            x[0, 3], x[1, K - 1], x[2, 0], x[3, :32] = math.nan, math.inf, -math.inf, 0
+            top = torch.tensor(448.0 if fmt == 8 else 6.0, dtype=t)
+            x[4, :64] = 0
+            x[4, 5], x[4, 40] = top, -torch.nextafter(top, 2 * top)          # the largest code, and a step above: the next scale
+        wide = torch.empty(rows, K + 16, dtype=t, device="cuda").normal_()
+        wide[:, 8:8 + K] = x.cuda()
+        codes = torch.full((rows + 1, Kp * fmt // 8), 0xA5, dtype=torch.uint8, device="cuda")
+        scales = torch.full((rows + 1, Kp // 32), 0xA5, dtype=torch.uint8, device="cuda")
+        assert wide[:, 8:].data_ptr() % 16 == 0
+        assert _lib.lib().dsv41_mx_quant(wide[:, 8:].data_ptr(), list(DT).index(dtype), rows, K, K + 16, fmt, Kp, codes.data_ptr(), scales.data_ptr(), None,
+                                         torch.cuda.current_stream().cuda_stream) == 0
+        assert (codes[rows] == 0xA5).all() and (scales[rows] == 0xA5).all()
+        codes, scales = codes[:rows].cpu(), scales[:rows].cpu()
+        bad = ~torch.isfinite(x.float()).reshape(rows, -1, 32).all(-1)
+        if fmt == 4:
+            code, byte, _ = ref_fp4(x)                                       # groups that are not finite: code 0, byte 255
+            want, zero = pack(code), 1
+        else:
+            ok = torch.where(bad.repeat_interleave(32, -1), torch.zeros((), dtype=t), x)
+            want, byte = (a.cpu() for a in quant.quant_fp8_e8m0(ok.float().cuda()))
+            q = ref_fp8(ok.double())
+            assert torch.equal(want.view(torch.float8_e4m3fn).double(), q[0]) and torch.equal(byte, q[1])
+            want[bad.repeat_interleave(32, -1)], byte[bad], zero = 0x7F, 255, 105   # 105: e of the floor, 1e-4 <= 448 * 2^-22
+        assert bad.sum() == (0 if rows <= 4 else 3)
+        n = K * fmt // 8
+        assert torch.equal(codes[:, :n], want) and not codes[:, n:].any()
+        assert torch.equal(scales[:, :K // 32], byte) and (scales[:, K // 32:] == zero).all()
