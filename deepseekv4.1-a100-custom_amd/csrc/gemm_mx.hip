@@ -64,10 +64,10 @@ __device__ __forceinline__ void spread() {
 // every wave and stage k + 1 is complete; the last step of stage k still has its matrix instructions to go, so they cover the reads behind
 // the barrier.
 //
-// Measured from codes: 8192 x 8192 x 8192 in 254 us for FP4 (4.3 PFLOP/s; the matrix instructions alone, on the same random codes, take 225:
-// the clock falls under them) and 366 us for FP8 (3.0 PFLOP/s of 4.0). 128 x 128 is bound by its rounds over the chip (2048 x 3328 x 7168, FP8:
-// 416 tiles on 512 places, 44 us), 64 x 64 by what a CU's LDS gives: 16 KB of copies and 32 KB of operands per 256 k (97 x 5120 x 8192, FP4:
-// 12.5 us).
+// Measured from codes (medians of a trace): 8192 x 8192 x 8192 in 262 us for FP4 (4.2 PFLOP/s; the matrix instructions alone, on the same random
+// codes, take 225: the clock falls under them) and 371 us for FP8 (3.0 PFLOP/s of 4.0). 128 x 128 is bound by its rounds over the chip (2048 x 3328 x
+// 7168, FP8: 416 tiles on 512 places, 43 us), 64 x 64 by what a CU's LDS gives: 16 KB of copies and 32 KB of operands per 256 k (97 x 5120 x 8192,
+// FP4: 12.4 us).
 template <int AF, int WM, int WT, int NT, int KP, int NS>
 struct Tile {
     static constexpr int RB = KP * (AF == 4 ? 64 : 128);       // bytes of a token row per stage
@@ -354,9 +354,11 @@ __device__ __forceinline__ void mx_gemm_tile(const MxArgs& a) {
 
     if constexpr (WM * WT == 1) {
         // K in parts: every wave leaves its sums in memory, and the last of a tile's waves in this place to arrive adds all parts in their order,
-        // its own among them. Nobody waits for anybody. The sums are stored and read at the device's scope, past the XCD's L2, so that their
-        // order around the counter's step needs no more than that the stores are done before it: a fence would write back the whole L2 for
-        // every wave (97 x 5120 x 8192 in three parts: 131 us).
+        // its own among them. Nobody waits for anybody. The sums are stored and read at the device's scope, past the XCD's L2. What orders them
+        // around the counter's step is that the stores have been acknowledged (the wait for vmcnt 0) before the counter moves, and that the loads
+        // are issued after its answer: how gfx950 carries out these instructions. The fences only keep the compiler's order; between workgroups
+        // the memory model would ask for a release and an acquire at the device's scope, which write back the whole L2 for every wave (97 x 5120 x
+        // 8192 in three parts: 131 us).
         if (a.split > 1) {
             float* const sums = a.part + ((long long)tile * a.split * NWV + wave) * 1024 + lane;   // part p: 1024 NWV p behind
             float* const mine = sums + (long long)part_k * NWV * 1024;
@@ -457,8 +459,8 @@ static int launch_tiles(const MxArgs& a, bool launch, hipStream_t st) {
 // streaming waves multiply their tiles (v_mfma_scale_f32_16x16x128_f8f6f4: 16 weight rows, up to 16 rows of x), and their sums are
 // added in wave order. Splitting the work by wave keeps the two streams' wait counters apart: a wave's loads complete in order, so
 // rows loaded behind the tiles would arrive with the last of them.
-// Measured with the rounding of x: 1 x 5120 x 8192 FP4 8.0 us (2.8 TB/s of weights: 2 us until the first arrive, 1 us of joins), 16 x 4608 x
-// 5120 FP8 9.9 us (7.2 from codes: every workgroup rounds all rows).
+// Measured with the rounding of x (medians of a trace): 1 x 5120 x 8192 FP4 8.2 us (2.7 TB/s of weights: 2 us until the first arrive, 1 us of joins,
+// 320 workgroups on 256 CUs), 16 x 4608 x 5120 FP8 10.6 us (8.1 from codes: every workgroup rounds all rows; 144 workgroups).
 // Lane (r = l % 16, q = l / 16) holds blocks 2 q and 2 q + 1 of a pair's eight in its two steps, so its two scale bytes are one half-word.
 #define SK_STREAM 8
 #define SK_QUANT 8

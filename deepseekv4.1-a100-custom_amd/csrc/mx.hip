@@ -46,7 +46,7 @@ struct Vec8 {
 
 // ------------------------------------------------------------------------------------------ quantiser
 // One lane takes eight values, four lanes a group; columns K .. Kp - 1 of the codes and scales are zero. One pass over x: the
-// stream of x and of what is written bounds it (32768 x 5120 bf16 with the values written too: 125 us, 6.1 TB/s; 16 x 5120: 2.8 us).
+// stream of x and of what is written bounds it (32768 x 5120 bf16 with the values written too: 126 us, 6.1 TB/s, without 74 us, 5.7; 16 x 5120: 2.8 us).
 template <int DT, int FMT, int VALUES>
 __global__ void __launch_bounds__(256) mx_quant_kernel(const void* __restrict__ x, long long ldx, long long rows, int K, int Kp,
                                                        uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, uint16_t* __restrict__ values) {
@@ -177,7 +177,7 @@ int mx_turn_scales(const uint8_t* xs, long long ldxs, int M, int K, uint8_t* out
 // The sums are fp32, and v goes to its codes without a rounding in between (y, where asked for, is v rounded to T). r is rounded to
 // the stream's type first because that is the value the next layer reads, and the statistics are of it.
 // One workgroup per row, the row in registers between the two passes over it; the row's bytes bound it (16384 x 5120 bf16 to FP8: 108 us,
-// 5.5 TB/s; one row, 3.4 us: latency).
+// 5.5 TB/s; to FP4 with y: 132 us, 5.4 TB/s; one row, 2.6 us: latency).
 template <int DT, int FMT, int T, int C>
 __global__ void __launch_bounds__(T) mx_norm_kernel(long long row0, const void* x, long long ldx, const void* res, long long ldr,
                                                     const void* __restrict__ g, float eps, double inv_k, int K, void* out, long long ldo, void* __restrict__ y,

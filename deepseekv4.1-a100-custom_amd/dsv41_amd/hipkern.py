@@ -446,11 +446,11 @@ def mx_plan(M: int, N: int, K: int, fmt: int):
     256 x 256, the one that takes least over the chip. Two tiles of plans 0 and 1 fit a CU, one of plan 2; the large ones go in rounds, the small
     ones follow each other evenly. Times per 128 k in us, from graph replays over weights larger than the last-level cache (us with the rounding
     of x, plan 0 / 1 / 2):
-      * FP4: 97 x 5120 x 8192 14.8 / 26.0 / 50.9, 512 x 4608 x 5120 23.5 / 26.7 / 40.4, 700 x 3999 x 2336 18.8 / 14.9 / 28.0, 1024 x 1280 x 5120
-        17.7 / 21.0 / 34.7, 2048 x 3328 x 7168 60.9 / 42.9 / 55.8, 2048 x 5120 x 8192 90.8 / 68.7 / 62.0, 8192 x 1280 x 5120 69.9 / 56.6 / 51.1
-      * FP8: 97 x 5120 x 8192 19.2 / 31.7 / 65.6, 512 x 4608 x 5120 31.6 / 27.2 / 48.8, 700 x 3999 x 2336 21.9 / 17.4 / 33.6, 1024 x 1280 x 5120
-        24.4 / 24.7 / 48.6, 2048 x 3328 x 7168 81.7 / 52.0 / 67.7, 2048 x 5120 x 8192 123.1 / 84.0 / 81.3, 8192 x 1280 x 5120 92.6 / 69.8 / 68.4
-    At worst 5 % over the best plan at these and twelve other sizes (64 x 32768 x 1280, FP4: 11.4 against 10.9)."""
+      * FP4: 97 x 5120 x 8192 15.2 / 26.2 / 51.2, 512 x 4608 x 5120 23.8 / 27.3 / 40.6, 700 x 3999 x 2336 16.8 / 14.3 / 27.4, 1024 x 1280 x 5120
+        18.2 / 21.2 / 34.8, 2048 x 3328 x 7168 60.2 / 43.0 / 55.3, 2048 x 5120 x 8192 91.4 / 68.6 / 62.0, 8192 x 1280 x 5120 69.9 / 57.7 / 51.8
+      * FP8: 97 x 5120 x 8192 19.6 / 32.1 / 65.8, 512 x 4608 x 5120 32.5 / 27.4 / 48.5, 700 x 3999 x 2336 20.5 / 17.2 / 33.0, 1024 x 1280 x 5120
+        24.8 / 25.0 / 48.8, 2048 x 3328 x 7168 83.2 / 53.0 / 67.4, 2048 x 5120 x 8192 127.0 / 83.9 / 80.2, 8192 x 1280 x 5120 93.1 / 69.2 / 67.2
+    At worst 5 % over the best plan at these and twelve other sizes (64 x 32768 x 1280: FP4 11.6 against 11.3, FP8 12.6 against 12.2)."""
     nk, Kp = -(-K // 256), -(-K // 128) * 128
     if M <= MX_ROWS and M * (nk * 32 * fmt + 16 + nk * 8 + 4) + 15 + 8192 <= 160 * 1024:
         return 3, 0
@@ -466,9 +466,10 @@ def mx_plan(M: int, N: int, K: int, fmt: int):
 def mx_parts(M: int, N: int, K: int, fmt: int) -> int:
     """Parts of K with which tiles of 64 x 64 are multiplied: as many as fill the chip's 256 CUs once, where each has stages of 256 k enough to
     pay for the join of its sums, 4 to 5 us (us with the rounding of x, whole / 2 / 3 / 4 parts; tiles):
-      * FP4: 33 x 5120 x 8192 (80) 14.5 / 13.1 / 13.1 / 16.0, 128 x 2048 x 16384 (64) 24.8 / 18.6 / 17.0 / 16.3, 64 x 4608 x 5120 (72)
-        12.7 / 12.0 / 11.9 / 14.5, 128 x 1280 x 5120 (40) 10.1 / 10.2 / 10.2 / 10.9, 97 x 5120 x 8192 (160) 15.2 / 18.0 / 17.7 / 21.2
-      * FP8: 18.5 / 15.2 / 14.2 / 16.9, 34.9 / 23.9 / 20.6 / 19.3, 16.2 / 13.5 / 12.6 / 15.7, 13.4 / 12.2 / 11.6 / 11.8, 19.4 / 20.2 / 19.2 / 23.7"""
+      * FP4: 33 x 5120 x 8192 (80) 14.6 / 13.6 / 13.2 / 16.1, 128 x 2048 x 16384 (64) 24.7 / 18.7 / 16.9 / 16.4, 64 x 4608 x 5120 (72)
+        12.7 / 11.9 / 11.8 / 14.5, 128 x 1280 x 5120 (40) 10.0 / 10.3 / 10.4 / 11.1, 97 x 5120 x 8192 (160) 15.3 / 17.7 / 17.5 / 21.2
+      * FP8: 18.3 / 14.9 / 14.2 / 17.0, 35.1 / 23.9 / 20.4 / 19.2, 16.0 / 13.4 / 12.5 / 15.7, 13.4 / 12.2 / 11.6 / 11.9, 19.7 / 20.2 / 19.4 / 24.0
+    (graph replays like mx_plan's, the same card)."""
     tiles, stages = -(-N // 64) * -(-M // 64), -(-K // 256)
     return max(1, min(4, 256 // tiles, stages // (12 if fmt == 4 else 6)))
 
