@@ -381,7 +381,7 @@ int dsv41_mx_quant(const void* x, int dtype, long long rows, int K, long long ld
 
 /* r = round(x + res) to dtype, into out (res NULL: r = x, out unused); v = r / sqrt(mean(r^2) + eps) * w in fp32; v quantised as
  * dsv41_mx_quant does (no rounding in between) into codes [rows][K fmt / 8] and scales [rows][K / 32]; y (optional, [rows][K]): v rounded
- * to dtype. out may be x or res itself. K % 32 == 0, 32 <= K <= 32768, 16-byte aligned rows. */
+ * to dtype. out may be x or res itself; it shares no byte with w, which is read after r is written, or else with x and res. K % 32 == 0, 32 <= K <= 32768, 16-byte aligned rows. */
 int dsv41_add_rmsnorm_mx(const void* x, long long ldx, const void* res, long long ldr, const void* w, float eps, int dtype, long long rows, int K,
                          int fmt, void* out, long long ldo, void* y, uint8_t* codes, uint8_t* scales, void* stream);
 
